@@ -1347,7 +1347,7 @@ static std::unordered_map<std::string, OpDef> &optable() {
   add("s_cbranch_execz", x_branch, C_BRANCH, B_EXECZ, "-");
   add("s_cbranch_execnz", x_branch, C_BRANCH, B_EXECNZ, "-");
   add("s_endpgm", x_endpgm, C_BRANCH, 0, "");
-  add("s_waitcnt s_nop s_waitcnt_vscnt s_waitcnt_depctr s_setprio s_inst_prefetch s_clause s_delay_alu s_set_gpr_idx_off s_setreg_b32 s_setreg_imm32_b32 s_icache_inv s_dcache_wb buffer_wbl2 buffer_inv s_dcache_inv", x_nop, C_WAIT, 0, "--");
+  add("s_waitcnt s_nop s_waitcnt_vscnt s_waitcnt_depctr s_setprio s_inst_prefetch s_clause s_delay_alu s_set_gpr_idx_off s_setreg_b32 s_setreg_imm32_b32 s_icache_inv buffer_wbl2 buffer_inv s_dcache_inv", x_nop, C_WAIT, 0, "--");
   add("s_sleep", x_sleep, C_WAIT, 0, "-");
   add("s_barrier", x_barrier, C_WAIT, 0, "");
   add("s_load_dword", x_sload, C_SMEM, 1, "bUu");

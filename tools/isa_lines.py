@@ -12,7 +12,7 @@ def classify(m):
     if m.startswith("v_"): return "valu"
     if m.startswith("ds_"): return "lds"
     if m.startswith(("global_", "buffer_", "flat_", "scratch_")): return "vmem"
-    if m.startswith(("s_load", "s_buffer_load", "s_store", "s_dcache")): return "smem"
+    if m.startswith(("s_load", "s_buffer_load")): return "smem"
     if m.startswith(("s_cbranch", "s_branch", "s_setpc", "s_call", "s_endpgm")): return "branch"
     if m.startswith(("s_waitcnt", "s_nop", "s_sleep", "s_barrier")): return "wait"
     if m.startswith("s_"): return "salu"
