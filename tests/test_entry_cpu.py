@@ -29,3 +29,8 @@ def test_build_compiles_the_reference_where_its_sources_are(monkeypatch, tmp_pat
     (tmp_path / "render.cc").write_text("")
     calls = commands_of_build(monkeypatch, tmp_path)
     assert [c for c, _ in calls] == ["library", "oracle", "ref"] and calls[2][1]["check"]
+
+
+def test_build_compiles_the_library_also_where_one_is_built(monkeypatch, tmp_path):
+    """build() answers whether the sources compile: a library left by an earlier build must not stand in for them."""
+    assert commands_of_build(monkeypatch, tmp_path)[0] == ("library", {"force": True})
