@@ -8,7 +8,7 @@ import pytest
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 SOURCE = re.compile(r"(\.(py|sh|hip|cc|c|cpp|hpp|h|s|S|inc|txt|cmake|mk)|/Makefile)$")
-# writes through the scalar data cache: scalar stores and atomics, that cache's write-back and discard; "s_dcache" alone is a prefix of them
+# writes through the scalar data cache: scalar stores and atomics, that cache's write-back and discard, and the bare prefix of the latter two
 SCALAR_CACHE_WRITE = re.compile(r"(?<![A-Za-z0-9_])s_(?:(?:scratch_|buffer_)?(?:store|atomic)|dcache(?:_wb|_discard|(?![a-z_])))")
 
 
