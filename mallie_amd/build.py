@@ -21,8 +21,10 @@ HEADERS = ["mgpu_device.hpp", "mgpu_kernels.hpp", "mgpu_sincos.hpp", "mgpu_enque
 # -ffile-prefix-map: __FILE__ (error messages) does not carry the checkout's path.  The binary still depends on that path
 # (clang's per-file ids of internal device symbols); rebuilt in the same place it is bit-identical, and bench.py matches the
 # committed PMC passes to it by its sha256 or, failing that, by source_digest() below
-FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-ffp-contract=off", "-fPIC", "-shared", "-Wall",
-         "-Wno-unused-function", "-ffile-prefix-map=%s=." % os.path.dirname(HERE)]
+# -packed-fp32-ops: no packed FP32 instruction (v_pk_add_f32 and its like), which hipcc -O3 makes of ordinary float code by itself and
+# some forms of which have given wrong results on the MI355X now and then.  (The host pass warns that it does not know the feature.)
+KERNEL_FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-ffp-contract=off", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+FLAGS = KERNEL_FLAGS + ["-fPIC", "-shared", "-Wall", "-Wno-unused-function", "-ffile-prefix-map=%s=." % os.path.dirname(HERE)]
 
 
 def hipcc():

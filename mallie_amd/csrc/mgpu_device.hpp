@@ -515,11 +515,10 @@ __device__ __forceinline__ bool leaf_hint_make(TriFn tri, uint32_t n, double wor
 // slots of the double form.
 // (The cone clauses are evaluated for every consulting lane, not only behind a missed box: six float FMAs against a second,
 // dependent trip to LDS in the middle of the step.)
-// Both boxes at once: the record's first twelve floats are stored INTERLEAVED -- (A.lo.x, B.lo.x), (A.lo.y, B.lo.y), (A.lo.z, B.lo.z),
-// (A.hi.x, B.hi.x), ... (leaf_hint_pack) -- so that the six subtractions and six multiplications of the two slab tests are six v_pk_add_f32 and
-// six v_pk_mul_f32 on the pairs as they were loaded (the origin and 1 / d broadcast by op_sel): the same IEEE operations on the same operands as
-// the one-box form, half the instructions (tools/isa_profile.py: -0.3 VALU wave-instructions per ray on C2).
-typedef float mgpu_f2 __attribute__((ext_vector_type(2)));
+// The record is stored INTERLEAVED -- (A.lo.x, B.lo.x), (A.lo.y, B.lo.y), (A.lo.z, B.lo.z), (A.hi.x, B.hi.x), ... (leaf_hint_pack): five
+// 16-byte LDS reads hold both boxes and both cones in any order, so the order costs nothing.  The two halves are evaluated one after the
+// other, a float at a time: the library is compiled without packed FP32 (mallie_amd/build.py), which would halve the issue slots of the
+// slab products and some forms of which have given wrong results on the MI355X.
 __device__ __forceinline__ void leaf_hint_pack(const float *rec, float *out) {
   for (int a = 0; a < 3; ++a) {
     out[2 * a] = rec[a];              // A.lo
@@ -533,28 +532,25 @@ __device__ __forceinline__ void leaf_hint_pack(const float *rec, float *out) {
   }
   for (int k = 20; k < kHintFloats; ++k) out[k] = rec[k];
 }
+__device__ __forceinline__ bool slab_hit_f32(float lx, float ly, float lz, float hx, float hy, float hz, float ox, float oy, float oz, float ix,
+                                             float iy, float iz, float bt_up) {
+  const float ax = (lx - ox) * ix, bx = (hx - ox) * ix, ay = (ly - oy) * iy, by = (hy - oy) * iy, az = (lz - oz) * iz, bz = (hz - oz) * iz;
+  const float tmin = __builtin_fmaxf(__builtin_fmaxf(__builtin_fminf(ax, bx), __builtin_fminf(ay, by)), __builtin_fminf(az, bz));
+  const float tmax = __builtin_fminf(__builtin_fminf(__builtin_fmaxf(ax, bx), __builtin_fmaxf(ay, by)), __builtin_fmaxf(az, bz));
+  return (tmax > 0.0f) && (tmin <= tmax) && (tmin <= bt_up);
+}
 __device__ __forceinline__ uint32_t leaf_hint_apply(float4 f0, float4 f1, float4 f2, float4 cA, float4 cB, uint32_t m, V3 org, V3 dir, double ix,
                                                     double iy, double iz, double bt, uint32_t &tri_cur, uint32_t &tri_end) {
   const float dx = (float)dir.x, dy = (float)dir.y, dz = (float)dir.z;
   const float ox = (float)org.x, oy = (float)org.y, oz = (float)org.z, jx = (float)ix, jy = (float)iy, jz = (float)iz;
   const float bt_up = __double2float_ru(bt);
-  // cA = (nbar_A.x, nbar_B.x, nbar_A.y, nbar_B.y), cB = (nbar_A.z, nbar_B.z, thr_A, thr_B): d . nbar of both halves in three packed operations
+  // cA = (nbar_A.x, nbar_B.x, nbar_A.y, nbar_B.y), cB = (nbar_A.z, nbar_B.z, thr_A, thr_B)
   // (NaN compares false: the half counts as grazed and stays)
-  const mgpu_f2 nx = {cA.x, cA.y}, ny = {cA.z, cA.w}, nz = {cB.x, cB.y};
-  const mgpu_f2 dn = __builtin_elementwise_fma(nx, (mgpu_f2){dx, dx}, __builtin_elementwise_fma(ny, (mgpu_f2){dy, dy}, nz * dz));
-  const bool sA = fabsf(dn[0]) >= cB.z;
-  const bool sB = fabsf(dn[1]) >= cB.w;
+  const bool sA = fabsf(__builtin_fmaf(dx, cA.x, __builtin_fmaf(dy, cA.z, dz * cB.x))) >= cB.z;
+  const bool sB = fabsf(__builtin_fmaf(dx, cA.y, __builtin_fmaf(dy, cA.w, dz * cB.y))) >= cB.w;
   // f0 = (A.lo.x, B.lo.x, A.lo.y, B.lo.y), f1 = (A.lo.z, B.lo.z, A.hi.x, B.hi.x), f2 = (A.hi.y, B.hi.y, A.hi.z, B.hi.z)
-  const mgpu_f2 lx = {f0.x, f0.y}, ly = {f0.z, f0.w}, lz = {f1.x, f1.y}, hx = {f1.z, f1.w}, hy = {f2.x, f2.y}, hz = {f2.z, f2.w};
-  const mgpu_f2 ax = (lx - ox) * jx, bx = (hx - ox) * jx, ay = (ly - oy) * jy, by = (hy - oy) * jy, az = (lz - oz) * jz, bz = (hz - oz) * jz;
-  bool hit[2];
-  for (int k = 0; k < 2; ++k) {
-    const float tmin = __builtin_fmaxf(__builtin_fmaxf(__builtin_fminf(ax[k], bx[k]), __builtin_fminf(ay[k], by[k])), __builtin_fminf(az[k], bz[k]));
-    const float tmax = __builtin_fminf(__builtin_fminf(__builtin_fmaxf(ax[k], bx[k]), __builtin_fmaxf(ay[k], by[k])), __builtin_fmaxf(az[k], bz[k]));
-    hit[k] = (tmax > 0.0f) && (tmin <= tmax) && (tmin <= bt_up);
-  }
-  const bool hA = !sA || hit[0];
-  const bool hB = !sB || hit[1];
+  const bool hA = !sA || slab_hit_f32(f0.x, f0.z, f1.x, f1.z, f2.x, f2.z, ox, oy, oz, jx, jy, jz, bt_up);
+  const bool hB = !sB || slab_hit_f32(f0.y, f0.w, f1.y, f1.w, f2.y, f2.w, ox, oy, oz, jx, jy, jz, bt_up);
   const uint32_t whole = tri_end - tri_cur, mid = tri_cur + m;
   if (!hB) tri_end = mid;
   if (!hA) tri_cur = hB ? mid : tri_end;

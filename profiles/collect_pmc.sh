@@ -24,7 +24,7 @@ for w in $wl; do
   done
 done
 # calibration: known byte counts (MI355X_MICROARCH.md, HBM: calibrate before trusting an absolute)
-if [ ! -x profiles/microbench/pmc_calib ]; then hipcc --offload-arch=gfx950 -O3 profiles/microbench/pmc_calib.hip -o profiles/microbench/pmc_calib > "$out/calib_build.log" 2>&1; fi
+if [ ! -x profiles/microbench/pmc_calib ]; then hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops profiles/microbench/pmc_calib.hip -o profiles/microbench/pmc_calib > "$out/calib_build.log" 2>&1; fi
 for pass in "fetch:FETCH_SIZE" "write:WRITE_SIZE"; do
   name=${pass%%:*}; ctr=${pass#*:}
   timeout 300 rocprofv3 --pmc $ctr --kernel-include-regex "k_calib" --output-format csv -d "$out/calib_$name" -o p -- profiles/microbench/pmc_calib > "$out/calib_$name.log" 2>&1

@@ -1,6 +1,6 @@
 // exact_cores.hip -- are sqrt_core / rcp_core (mgpu_device.hpp: the compiler's own fp64 sqrt / division expansions without
 // their range-scaling and special-case steps) bit-identical to sqrt(x) / (1.0 / x) on the ranges the kernels use them on?
-// build: hipcc --offload-arch=gfx950 -O3 -ffp-contract=off -I mallie_amd/csrc -o exact_cores profiles/microbench/exact_cores.hip
+// build: hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -ffp-contract=off -I mallie_amd/csrc -o exact_cores profiles/microbench/exact_cores.hip
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 #include <stdio.h>

@@ -1,5 +1,5 @@
 // mailbox_latency.hip -- what one host -> resident kernel -> host round trip costs, by where the request word lives.
-//   hipcc --offload-arch=gfx950 -O3 mailbox_latency.hip -o mailbox_latency && ./mailbox_latency
+//   hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops mailbox_latency.hip -o mailbox_latency && ./mailbox_latency
 // A resident wave polls a request word and answers by writing an acknowledgement word into host memory the device maps; the host
 // writes the next request as soon as it sees the answer.  (a) request word in mapped host memory: the device's poll is a PCIe read;
 // (b) request word in device memory the host writes through the BAR (fine-grained allocation), the device polls its own HBM.

@@ -6,7 +6,7 @@
 //   k_calib_write12  every lane writes three dwords at 12-byte pitch, all lanes of a wave at once: the stores of
 //                    k_render_sm's radiance planes (one pixel = 12 bytes, tile-major) when a whole tile lands together
 //                                                                                                        -> 0.75 GiB written
-// Build: hipcc --offload-arch=gfx950 -O3 profiles/microbench/pmc_calib.hip -o profiles/microbench/pmc_calib
+// Build: hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops profiles/microbench/pmc_calib.hip -o profiles/microbench/pmc_calib
 // Run:   rocprofv3 --pmc FETCH_SIZE -- profiles/microbench/pmc_calib      (and again with WRITE_SIZE)
 #include <hip/hip_runtime.h>
 #include <cstdio>

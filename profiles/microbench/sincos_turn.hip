@@ -2,7 +2,7 @@
 // (mgpu_device.hpp): the nearest of 64 tabulated angles (the table is filled with the device library's sincospi at kernel
 // start) plus a remainder |r| <= 1/64 of a half turn through two four-term series, combined by the addition theorem.
 // This program compares it with sincospi(2 * k / 2^32) for EVERY k: maximal absolute difference and the maximal difference
-// in units of 2^-53 (the spacing of doubles just below 1).  Build: hipcc --offload-arch=gfx950 -O3 -ffp-contract=off
+// in units of 2^-53 (the spacing of doubles just below 1).  Build: hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -ffp-contract=off
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <cstdint>

@@ -7,6 +7,8 @@ usage: python tools/isa_lines.py <file.hip> '<demangled kernel substring>' [--to
   --ranges: line ranges of the MAIN file to sum under a name (e.g. 372-451:NODE,452-604:TRI,605-1043:SHADE); lines of other files are
   summed per file and function-sized range automatically (per 'file:line' otherwise)."""
 import collections, os, re, subprocess, sys, tempfile
+sys.path.insert(0, os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
+from mallie_amd.build import KERNEL_FLAGS
 
 def classify(m):
     if m.startswith("v_"): return "valu"
@@ -31,7 +33,7 @@ def main():
     defs = [x for x in a if x.startswith("-D")]
     with tempfile.TemporaryDirectory() as tmp:
         out = os.path.join(tmp, "k.s")
-        subprocess.run(["/opt/rocm/bin/hipcc", "--offload-arch=gfx950", "-O3", "-std=c++17", "-ffp-contract=off", "-S", "--cuda-device-only", "-gline-tables-only",
+        subprocess.run(["/opt/rocm/bin/hipcc"] + KERNEL_FLAGS + ["-S", "--cuda-device-only", "-gline-tables-only",
                         src, "-o", out] + defs, check=True, capture_output=True)
         lines = open(out).read().split("\n")
     files = {}

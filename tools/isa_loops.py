@@ -6,6 +6,8 @@ its inner loops) give the instructions one trip can issue at most.  With -gline-
 Classes as rocprofv3's SQ_INSTS_* count them (VALU, SALU without waitcnt / nop / branches, branch, LDS, VMEM, SMEM).
 usage: python tools/isa_loops.py <file.hip> '<demangled kernel substring>' [-D...]"""
 import collections, os, re, subprocess, sys, tempfile
+sys.path.insert(0, os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
+from mallie_amd.build import KERNEL_FLAGS
 
 
 def classify(m):
@@ -22,7 +24,7 @@ def classify(m):
 def analyse(src, kern, defs=()):
     with tempfile.TemporaryDirectory() as tmp:
         out = os.path.join(tmp, "k.s")
-        subprocess.run(["/opt/rocm/bin/hipcc", "--offload-arch=gfx950", "-O3", "-std=c++17", "-ffp-contract=off", "-S", "--cuda-device-only", "-gline-tables-only",
+        subprocess.run(["/opt/rocm/bin/hipcc"] + KERNEL_FLAGS + ["-S", "--cuda-device-only", "-gline-tables-only",
                         src, "-o", out] + list(defs), check=True, capture_output=True)
         lines = open(out).read().split("\n")
     files = {}

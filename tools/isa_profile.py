@@ -9,6 +9,8 @@ usage: python tools/isa_profile.py c2|c4|... [W H spp] [--src mgpu_render_sm.hip
 import collections, json, os, re, subprocess, sys, tempfile
 R = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 CSRC = os.path.join(R, "mallie_amd", "csrc")
+sys.path.insert(0, R)
+from mallie_amd.build import KERNEL_FLAGS
 # bodies of k_render_sm's wave loop by line range of mgpu_render_sm.hip (kept next to the source: tools/isa_profile.py --check-ranges prints the lines)
 MARKERS = [("prologue", r"__global__ __launch_bounds__"), ("scheduler", r"^  for \(;;\) \{$"), ("NODE step", r"=+ NODE step =+"), ("TRI step", r"=+ TRI step =+"),
            ("SHADE: finish the ray", r"=+ SHADE step =+"), ("SHADE: path hand-out", r"---- \(2\) path hand-out"), ("SHADE: start path / arm ray", r"---- \(3\) next path / next traversal"),
@@ -51,7 +53,7 @@ def main():
         for s in srcs:
             out = os.path.join(tmp, s.replace(".hip", ".s"))
             dumps.append(out)
-            procs.append(subprocess.Popen(["/opt/rocm/bin/hipcc", "--offload-arch=gfx950", "-O3", "-std=c++17", "-ffp-contract=off", "-S", "--cuda-device-only", "-gline-tables-only",
+            procs.append(subprocess.Popen(["/opt/rocm/bin/hipcc"] + KERNEL_FLAGS + ["-S", "--cuda-device-only", "-gline-tables-only",
                                            os.path.join(CSRC, s), "-o", out] + defs, stderr=subprocess.DEVNULL))
         for p in procs:
             if p.wait() != 0:

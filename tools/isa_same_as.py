@@ -4,13 +4,15 @@ trees with hipcc -S for gfx950 and compares the instruction streams (labels, sym
 usage: python tools/isa_same_as.py <commit> [file.hip ...]     (round 5: 9fdbfd3, the last commit the GPU suite ran on)"""
 import os, re, subprocess, sys, tempfile
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+sys.path.insert(0, ROOT)
+from mallie_amd.build import KERNEL_FLAGS
 commit = sys.argv[1]
 files = sys.argv[2:] or [f for f in sorted(os.listdir(os.path.join(ROOT, "mallie_amd", "csrc"))) if f.endswith(".hip")]
 
 
 def stream(src):
     with tempfile.NamedTemporaryFile(suffix=".s") as t:
-        r = subprocess.run(["/opt/rocm/bin/hipcc", "--offload-arch=gfx950", "-O3", "-std=c++17", "-ffp-contract=off", "-S", "--cuda-device-only", "-o", t.name, src],
+        r = subprocess.run(["/opt/rocm/bin/hipcc"] + KERNEL_FLAGS + ["-S", "--cuda-device-only", "-o", t.name, src],
                            capture_output=True, text=True)
         if r.returncode:
             return None

@@ -1,9 +1,11 @@
 #!/usr/bin/env python3
 """Register / spill / LDS table of every kernel in a .hip file (hipcc -Rpass-analysis=kernel-resource-usage).
 usage: python tools/kernel_resources.py mallie_amd/csrc/mgpu_render_sm.hip [extra -D flags]"""
-import re, subprocess, sys
+import os, re, subprocess, sys
+sys.path.insert(0, os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
+from mallie_amd.build import KERNEL_FLAGS
 src, extra = sys.argv[1], sys.argv[2:]
-cmd = ["/opt/rocm/bin/hipcc", "--offload-arch=gfx950", "-O3", "-std=c++17", "-ffp-contract=off", "-c",
+cmd = ["/opt/rocm/bin/hipcc"] + KERNEL_FLAGS + ["-c",
        "-Rpass-analysis=kernel-resource-usage", src, "-o", "/dev/null"] + extra
 err = subprocess.run(cmd, capture_output=True, text=True).stderr
 rows, cur = [], None
